@@ -13,7 +13,6 @@ listed() and draw() give cases as dicts of plain values, prepare() a case's inpu
 torch where `own` is false, through the package's entry points where it is true. work() is what a pass cannot do
 without, exact() the same outputs in 64 bits.
 """
-import functools
 import math
 import random
 import sys
@@ -31,9 +30,8 @@ DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
 PKG = Path(__file__).resolve().parents[1] / "rumik-fast_amd"
 
 
-@functools.cache
 def _modules():
-    """the package's modules, imported by name as its users do, once"""
+    """the package's modules, imported by name as its users do"""
     for p in (PKG / "kernels", PKG / "engine"):
         if str(p) not in sys.path:
             sys.path.insert(0, str(p))
