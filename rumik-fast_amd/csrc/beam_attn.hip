@@ -184,11 +184,14 @@ RK_DEV void scale_weights(float (&vw)[8], State<RT>& s) {
 }
 
 // The weights of tile r's query rows for the quad's eight slots, from their dot products; the running maximum, the sum
-// and, when the maximum moves, acc follow. ok: bit i set where slot i is one. The sum is of the rounded weights, those
+// and, when the maximum moves, acc follow. A score is the rounded product fl(t qs) in the maximum and in the exponent
+// alike: fused into the subtraction, the highest score's exponent would be its product's rounding error, half a step of the
+// maximum (32 at 2^29), and no longer 0. ok: bit i set where slot i is one. The sum is of the rounded weights, those
 // that meet V, by one more product with ones (the VALU is the busier unit); int8's weights meet V with its scales in them,
 // there it is of the fp32 ones.
 template <bool BF16, bool Q8, bool MASK, int RT>
 RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)[8], uint32_t ok, State<RT>& s, int r) {
+#pragma clang fp contract(off)
     float t[8];
     float top = kLowest;
 #pragma unroll
@@ -209,8 +212,8 @@ RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float x = __builtin_fmaf(t[i], s.qs[r], -s.m[r]);
-        t[i] = __builtin_amdgcn_exp2f(MASK && !(ok >> i & 1) ? -INFINITY : x);
+        const float x = t[i] * s.qs[r];
+        t[i] = __builtin_amdgcn_exp2f(MASK && !(ok >> i & 1) ? -INFINITY : x - s.m[r]);
     }
     u4_t w;
     if constexpr (Q8) {

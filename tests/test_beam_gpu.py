@@ -543,6 +543,42 @@ def test_attn_large_sizes_of_the_type(dev):
     check_attn(c["o"], c["q"], lambda b, h: (kd[0], vd[0, :66]), BF16, c["scale"] / big ** 2, c["unit"])
 
 
+# paths of an attention call: one launch; split, with a join; the prefix tile by tile (plain; plain and int8)
+PATHS = [(3, 2, 4, 100, 40), (3, 2, 4, 700, 300), (200, 8, 1, 2500, 40), (200, 8, 1, 10500, 40)]
+
+
+def dense(c, *index):
+    """a cache's values in float64, at the given index"""
+    return (c[0].double() * c[1].double()[..., None] if isinstance(c, tuple) else c.double())[index]
+
+
+@pytest.mark.parametrize("dt,p8,s8", KINDS)
+@pytest.mark.parametrize("B,nkv,rep,S,T", PATHS)
+def test_attn_large_scores(dt, p8, s8, B, nkv, rep, S, T, dev):
+    """Scores of 2^29 and more (bf16: 2^83), of which an fp32 holds no fraction: a few slots of the one highest score share
+    the row, wherever they lie. Every product here is exact, so the weights are, but for their rounding to 16 bits."""
+    unit = 2.0 ** (13 if dt is F16 else 40)
+    plen, slen = S - 1, T - 1
+    c = attn_case(dev, dt, B, nkv, rep, S, T, plen, [slen - 1], p8, s8, seed=S, junk=0.0)
+    size = unit * (1 + torch.arange(B * nkv * rep, device=dev) % 16 / 16)
+    c["q"].copy_(size[:, None].expand(-1, HD).reshape(B, -1))
+    tops, stops = sorted({0, 33, S // 2, S - 2}), [T // 2, T - 2]
+    for cache, at, n in ((c["kc"], tops, plen), (c["ks"], stops, slen)):
+        rows, of = (cache[0], 32) if isinstance(cache, tuple) else (cache, unit / 2)
+        rows.fill_(of)
+        rows[..., at, :] = 2 * of
+        rows[..., n:, :] = 3 * of if of == 32 else 1.5 * unit  # behind the length
+        if of == 32:
+            cache[1].fill_(unit / 64)
+    v = torch.cat((dense(c["vc"])[:, tops].expand(B, -1, -1, -1), dense(c["vs"])[:, :, stops]), 2)
+    want, mag = (x.mean(2).repeat_interleave(rep, 1).reshape(B, -1) for x in (v, v.abs()))
+    for sign in (1, -1):
+        q = c["q"] * sign
+        beam.attn(q, c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], sign * c["scale"])
+        off = (c["o"].double() - want).abs()
+        assert bool((off <= (2 * U[dt] + 2.0 ** -20) * mag + U[dt] * want.abs() + 1e-7).all()), float((off / mag).max())
+
+
 @pytest.mark.parametrize("p8", [False, True])
 def test_attn_matches_the_one_row_attention(p8, dev):
     """A hypothesis by itself is fused.attn over one cache holding its prefix and suffix."""
