@@ -185,7 +185,7 @@ RK_DEV void scale_weights(float (&vw)[8], State<RT>& s) {
 
 // The weights of tile r's query rows for the quad's eight slots, from their dot products; the running maximum, the sum
 // and, when the maximum moves, acc follow. A score is the rounded product fl(t qs) in the maximum and in the exponent
-// alike: fused into the subtraction, the highest score's exponent would be its product's rounding error, half a step of the
+// alike; fused into the subtraction, the highest score's exponent would be its product's rounding error, half a step of the
 // maximum (32 at 2^29), and no longer 0. ok: bit i set where slot i is one. The sum is of the rounded weights, those
 // that meet V, by one more product with ones (the VALU is the busier unit); int8's weights meet V with its scales in them,
 // there it is of the fp32 ones.
@@ -193,15 +193,15 @@ template <bool BF16, bool Q8, bool MASK, int RT>
 RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)[8], uint32_t ok, State<RT>& s, int r) {
 #pragma clang fp contract(off)
     float t[8];
-    float top = kLowest;
+    float top = kLowest;  // as it is, no product of it: a lane without a slot is below any score
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         t[i] = sc[i >> 2][i & 3];
         if constexpr (Q8) t[i] *= ks[i];
+        t[i] *= s.qs[r];
         if constexpr (MASK) t[i] = ok >> i & 1 ? t[i] : -INFINITY;
         top = fmaxf(top, t[i]);
     }
-    top *= s.qs[r];
     if (__ballot(top > s.m[r] + kSlack)) {  // some row's maximum moved by more than 2^kSlack
         top = max_xor<32>(max_xor<16>(top));
         const float mn = fmaxf(s.m[r], top), f = __builtin_amdgcn_exp2f(s.m[r] - mn);
@@ -211,10 +211,7 @@ RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)
         for (int d = 0; d < 8; ++d) s.acc[r][d] *= f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = t[i] * s.qs[r];
-        t[i] = __builtin_amdgcn_exp2f(MASK && !(ok >> i & 1) ? -INFINITY : x - s.m[r]);
-    }
+    for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(t[i] - s.m[r]);
     u4_t w;
     if constexpr (Q8) {
         float sum = 0.f;

@@ -579,6 +579,22 @@ def test_attn_large_scores(dt, p8, s8, B, nkv, rep, S, T, dev):
         assert bool((off <= (2 * U[dt] + 2.0 ** -20) * mag + U[dt] * want.abs() + 1e-7).all()), float((off / mag).max())
 
 
+@pytest.mark.parametrize("S,T", [(60, 30), (400, 140)])
+def test_attn_no_slot_beside_low_scores(S, T, dev):
+    """A suffix whose table leads to no slot does not count as a score, however small the scale: scores of about -256 beside
+    it, keys near the end of bf16's range."""
+    c = attn_case(dev, BF16, 2, 1, 2, S, T, S - 3, [T - 1], False, True, table=np.full((2, T), -1), seed=S, sharp=1.0,
+                  junk=0.0)
+    q = c["q"].view(2, 2, HD)
+    q[..., :16] = 16.0
+    c["kc"].mul_(2.0 ** 116)
+    c["kc"][..., :16] = -2.0 ** 118
+    c["scale"] = 2.0 ** -118
+    beam.attn(c["q"], c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], c["scale"], src=c["src"])
+    kd, vd = (c[k][0, :S - 3].double().cpu().numpy() for k in ("kc", "vc"))
+    check_attn(c["o"], c["q"], lambda b, h: (kd, vd), BF16, c["scale"], c["unit"])
+
+
 @pytest.mark.parametrize("p8", [False, True])
 def test_attn_matches_the_one_row_attention(p8, dev):
     """A hypothesis by itself is fused.attn over one cache holding its prefix and suffix."""
