@@ -202,7 +202,8 @@ RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)
         if constexpr (MASK) t[i] = ok >> i & 1 ? t[i] : -INFINITY;
         top = fmaxf(top, t[i]);
     }
-    if (__ballot(top > s.m[r] + kSlack)) {  // some row's maximum moved by more than 2^kSlack
+    // some row's maximum moved by more than 2^kSlack (their difference: s.m + kSlack may round up to the next score)
+    if (__ballot(top - s.m[r] > kSlack)) {
         top = max_xor<32>(max_xor<16>(top));
         const float mn = fmaxf(s.m[r], top), f = __builtin_amdgcn_exp2f(s.m[r] - mn);
         s.m[r] = mn;

@@ -547,6 +547,26 @@ def test_attn_large_sizes_of_the_type(dev):
 PATHS = [(3, 2, 4, 100, 40), (3, 2, 4, 700, 300), (200, 8, 1, 2500, 40), (200, 8, 1, 10500, 40)]
 
 
+def attend64(q, kv, suffix, scale):
+    """softmax(scale q . k) v and sum w |v| beside it in float64, [B, NH, HD]: q [B, NH * HD] over the prefix rows kv = (k, v)
+    [nkv, n, HD] and each hypothesis's own suffix = (k, v) [B, nkv, m, HD], all of them slots"""
+    kd, vd = (x.double() for x in kv)
+    ks, vs = (x.double() for x in suffix)
+    nkv = kd.shape[0]
+    qd = q.double().view(q.shape[0], nkv, -1, HD)
+    sp = (qd[:, :, :, None] * kd[None, :, None]).sum(-1) if kd.shape[1] < 1000 else \
+        torch.stack([qd[:, g] @ kd[g].t() for g in range(nkv)], 1)
+    s = torch.cat((sp, (qd[:, :, :, None] * ks[:, :, None]).sum(-1)), -1) * scale
+    w = torch.exp(s - s.amax(-1, keepdim=True))
+    w = w / w.sum(-1, keepdim=True)
+    n = kd.shape[1]
+    both = []
+    for x, y in ((vd, vs), (vd.abs(), vs.abs())):
+        o = torch.stack([w[:, g, :, :n] @ x[g] for g in range(nkv)], 1) + (w[..., n:, None] * y[:, :, None]).sum(-2)
+        both.append(o.flatten(1, 2))
+    return both
+
+
 def dense(c, *index):
     """a cache's values in float64, at the given index"""
     return (c[0].double() * c[1].double()[..., None] if isinstance(c, tuple) else c.double())[index]
@@ -577,6 +597,33 @@ def test_attn_large_scores(dt, p8, s8, B, nkv, rep, S, T, dev):
         beam.attn(q, c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], sign * c["scale"])
         off = (c["o"].double() - want).abs()
         assert bool((off <= (2 * U[dt] + 2.0 ** -20) * mag + U[dt] * want.abs() + 1e-7).all()), float((off / mag).max())
+
+
+@pytest.mark.parametrize("dt,p8,s8", KINDS)
+@pytest.mark.parametrize("B,nkv,rep,S,T", [(64, 2, 1, 600, 100), (64, 4, 1, 300, 700), (3, 2, 4, 40000, 4),
+                                           (200, 8, 1, 2500, 4), (200, 8, 1, 10500, 4)])
+def test_attn_large_scores_that_rise(dt, p8, s8, B, nkv, rep, S, T, dev):
+    """Scores around 2^27, where fp32 has every 16th number, that rise from 2^27 + 16 to the next one while a wave goes on;
+    exactly so, in log2 units, by this scale."""
+    scale = float(np.float32(math.log(2)))
+    assert np.float32(scale) * np.float32(1.4426950408889634) == 1
+    c = attn_case(dev, dt, B, nkv, rep, S, T, S - 1, [T - 2], p8, s8, seed=S, junk=0.0)
+    c["q"].zero_()
+    c["q"].view(B, -1, HD)[..., 0], c["q"].view(B, -1, HD)[..., 1] = 2.0 ** 12, 2.0 ** -5
+    for k in (c["kc"], c["ks"]):
+        rows, unit = (k[0], 1) if isinstance(k, tuple) else (k, 512)
+        n = rows.shape[-2]
+        rows.zero_()
+        rows[..., 0] = 64 * unit
+        rows[..., 1] = 1 * unit
+        rows[..., n * 6 // 10:, 1] = 2 * unit
+        if unit == 1:
+            k[1].fill_(512.0)
+    beam.attn(c["q"], c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], scale)
+    want, mag = attend64(c["q"], [dense(c[k])[:, :S - 1] for k in ("kc", "vc")],
+                         [dense(c[k])[:, :, :T - 1] for k in ("ks", "vs")], scale)
+    off = (c["o"].double().view_as(want) - want).abs()
+    assert bool((off <= (2 * U[dt] + 2.0 ** -17) * mag + U[dt] * want.abs() + 1e-7).all()), float((off / mag).max())
 
 
 @pytest.mark.parametrize("S,T", [(60, 30), (400, 140)])
