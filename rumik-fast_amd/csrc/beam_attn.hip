@@ -7,8 +7,8 @@
 // the order 4 quad + (0..3), 16 + 4 quad + (0..3): the weights stay in their lanes. The softmax is in log2 units with a
 // running maximum that moves only when a score exceeds it by more than 2^kSlack, so the exchange between the quads and
 // the rescaling of O run in few steps. Scores, statistics and sums are fp32. P is rounded to the operands' type (fp16:
-// 2^-11, bf16: 2^-8 relative, as much again as the output's own rounding). int8 caches run on fp16 operands, in which the
-// codes are exact; K's scale goes to the scores, V's scale to P.
+// 2^-11 relative, or 2^-32 of the largest weight where that is more, bf16: 2^-8 relative; as much again as the output's own
+// rounding). int8 caches run on fp16 operands, in which the codes are exact; K's scale goes to the scores, V's scale to P.
 //
 // Launches: direct_kernel alone for small caches; else part_kernel for the suffixes and short prefixes, wide_kernel for
 // long prefixes of many query rows and join_kernel, which adds the splits up. All read the lengths on the device; a
@@ -99,13 +99,17 @@ template <int RT>
 struct State {
     u4_t q[RT][4];       // B operand of K Q: the row's dims in K's order
     float qs[RT];        // |scale| * log2(e) (int8 with bf16: times what the fp16 copy of q was divided by)
-    float m[RT];         // running maximum in log2 units (at most kSlack below the true one)
+    float m[RT];         // running maximum in log2 units, kLift below (at most kLift + kSlack below the true one)
     f4_t l[RT];          // sum of weights in l[.][0]; int8: of the quad's weights
     f4_t acc[RT][8];     // sum of weights * V, dim 8 (4 quad + e) + d in acc[.][d][e]
     float cap;           // int8: a power of two that no V scale so far exceeds; acc is in units of cap / 2^kHead
 };
 constexpr float kSlack = 8.0f;
 constexpr int kHead = 7;
+// What the maximum's weight is lifted by: a plain fp16 cache's weights meet V in fp16, which has no more than 2^-25 below
+// 1. Lifted, they reach from 2^(kSlack + 7) = 2^15 down to 2^-32 of the maximum's weight. int8 has kHead for that.
+template <bool BF16, bool Q8>
+constexpr float kLift = BF16 || Q8 ? 0.0f : 7.0f;
 constexpr float kLowest = -3.402823466e38f;  // "no maximum yet": exp2(-inf - kLowest) is 0, not NaN
 
 // The state before the first slot. qrow: this lane's query row of tile r, its 128 values. CODES: K's order of dims is 64
@@ -202,10 +206,11 @@ RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)
         if constexpr (MASK) t[i] = ok >> i & 1 ? t[i] : -INFINITY;
         top = fmaxf(top, t[i]);
     }
+    constexpr float lift = kLift<BF16, Q8>;
     // some row's maximum moved by more than 2^kSlack (their difference: s.m + kSlack may round up to the next score)
-    if (__ballot(top - s.m[r] > kSlack)) {
+    if (__ballot(top - s.m[r] > kSlack + lift)) {
         top = max_xor<32>(max_xor<16>(top));
-        const float mn = fmaxf(s.m[r], top), f = __builtin_amdgcn_exp2f(s.m[r] - mn);
+        const float mn = fmaxf(s.m[r], top - lift), f = __builtin_amdgcn_exp2f(s.m[r] - mn);
         s.m[r] = mn;
         s.l[r] *= f;
 #pragma unroll

@@ -642,6 +642,40 @@ def test_attn_no_slot_beside_low_scores(S, T, dev):
     check_attn(c["o"], c["q"], lambda b, h: (kd, vd), BF16, c["scale"], c["unit"])
 
 
+@pytest.mark.parametrize("dt,p8,s8", KINDS)
+@pytest.mark.parametrize("B,nkv,rep,S,T", PATHS)
+@pytest.mark.parametrize("depth", [12.0, 16.203125, 17.40625, 20.0])
+def test_attn_many_low_weights(dt, p8, s8, B, nkv, rep, S, T, depth, dev):
+    """One slot leads by `depth`, all others have the same score: in the dims where the leading one's V is 0 the others are
+    the result. A weight is held to within 2^-32 of the largest one (half a step of fp16 below 2^7), int8: 2^-31 with V's
+    scale in it, besides its rounding."""
+    plen, slen = S - 1, T - 1
+    c = attn_case(dev, dt, B, nkv, rep, S, T, plen, [slen - 1], p8, s8, seed=S, junk=0.0)
+    g = torch.Generator(device=dev).manual_seed(S)
+    c["q"].zero_()
+    c["q"].view(B, -1, HD)[..., 0] = 1.0
+    v = (torch.rand(nkv, S, HD, device=dev, generator=g) + 1) * 1024
+    v[:, 0, 64:] = 0
+    vs = (torch.rand(B, nkv, T, HD, device=dev, generator=g) + 1) * 1024
+    c["vc"], c["vs"] = as_cache(v.to(dt), p8)[0], as_cache(vs.to(dt), s8)[0]
+    for k in (c["kc"], c["ks"]):
+        (k[0] if isinstance(k, tuple) else k).zero_()
+    top = torch.tensor(depth, dtype=dt).item()
+    if p8:
+        c["kc"][0][:, 0, 0] = 64
+        c["kc"][1][:, 0] = top / 64
+    else:
+        c["kc"][:, 0, 0] = top
+    beam.attn(c["q"], c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], 1.0)
+    want, mag = attend64(c["q"], [dense(c[k])[:, :plen] for k in ("kc", "vc")],
+                         [dense(c[k])[:, :, :slen] for k in ("ks", "vs")], 1.0)
+    n, vmax = plen + slen, 2048 * (1 + 2.0 ** -8)
+    grid = 2.0 ** (-31 if p8 or s8 else -32) * (127.5 if p8 or s8 else 1)  # int8: of the largest V scale, for codes to 127
+    tol = 2 * (U[dt] + 2.0 ** -18) * mag + n * grid * (vmax / 127 if p8 or s8 else vmax) + U[dt] * want.abs() + 2.0 ** -25
+    off = (c["o"].double().view_as(want) - want).abs()
+    assert bool((off <= tol).all()), (float((off / tol).max()), float((off / mag).max()))
+
+
 @pytest.mark.parametrize("p8", [False, True])
 def test_attn_matches_the_one_row_attention(p8, dev):
     """A hypothesis by itself is fused.attn over one cache holding its prefix and suffix."""
