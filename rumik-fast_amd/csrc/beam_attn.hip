@@ -590,11 +590,25 @@ struct Tile {
     static constexpr int kLds = kCount * kBytes + (Q8 ? 4 * kPlain : 0);
 };
 
-// s_waitcnt vmcnt(n) alone (bits [3:0] and [15:14]; expcnt and lgkmcnt at their maxima)
-#define RK_VMCNT(n) __builtin_amdgcn_s_waitcnt(((n) & 15) | (((n) >> 4) << 14) | (7 << 4) | (15 << 8))
-
-// lgkmcnt(0) alone
-#define RK_LGKMCNT0() __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8))
+// Waits and barriers of the ring. To the compiler the builtins are no memory operations: the fences (no instruction) keep
+// LDS reads and copies on their side of them.
+RK_DEV void fence() { asm volatile("" ::: "memory"); }
+template <int N>
+RK_DEV void wait_copies() {  // s_waitcnt vmcnt(N) alone (bits [3:0] and [15:14]; expcnt and lgkmcnt at their maxima)
+    fence();
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+    fence();
+}
+RK_DEV void wait_lds() {  // lgkmcnt(0) alone
+    fence();
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+    fence();
+}
+RK_DEV void barrier() {
+    fence();
+    __builtin_amdgcn_s_barrier();
+    fence();
+}
 
 template <bool BF16, bool Q8, int RT, int RW>
 __global__ __launch_bounds__(128 * RW, RW > 2 ? 2 : 1) void wide_kernel(AttnArgs a) {
@@ -714,10 +728,7 @@ __global__ __launch_bounds__(128 * RW, RW > 2 ? 2 : 1) void wide_kernel(AttnArgs
         }
     };
     auto converted = [&] {
-        if constexpr (Q8) {
-            RK_LGKMCNT0();
-            asm volatile("" ::: "memory");
-        }
+        if constexpr (Q8) wait_lds();
     };
     // The two waves of a SIMD, one of each half, work in opposite phases: while one multiplies (the last tile's weights
     // with its V, then q with this tile's K) the other is in its softmax, so that the matrix cores and the VALU are both
@@ -763,15 +774,14 @@ __global__ __launch_bounds__(128 * RW, RW > 2 ? 2 : 1) void wide_kernel(AttnArgs
         }
         if constexpr (!Q8) read_k(i + 1);
         softmax<BF16, Q8, MASK>(st, sc, s, w);
-        RK_LGKMCNT0();  // V's and K's reads have ended before the barrier
+        wait_lds();  // V's and K's reads have ended before the barrier
     };
-    auto landed = [&] { RK_VMCNT((TL::kCount - 3) * kPerTile); };
+    auto landed = [&] { wait_copies<(TL::kCount - 3) * kPerTile>(); };
     auto phase = [&] {
         if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        if constexpr (Q8) asm volatile("" ::: "memory");
+        barrier();
     };
-    RK_VMCNT((TL::kCount - (Q8 ? 2 : 1)) * kPerTile);
+    wait_copies<(TL::kCount - (Q8 ? 2 : 1)) * kPerTile>();
     phase();
     if constexpr (Q8) {
         convert(0);
@@ -818,7 +828,7 @@ __global__ __launch_bounds__(128 * RW, RW > 2 ? 2 : 1) void wide_kernel(AttnArgs
         phase();
     }
     add_values<kB, false, true>(st, w, s);
-    RK_VMCNT(0);  // the copies past the last tile have landed too, before other data takes their place
+    wait_copies<0>();  // the copies past the last tile have landed too, before other data takes their place
     __syncthreads();
     f4_t* sums = reinterpret_cast<f4_t*>(ring) + rw * RT * 8 * 64 + lane;
     f4_t* rows = reinterpret_cast<f4_t*>(ring) + (RW * RT + wave) * 8 * 64;  // this wave's 16 rows of 128
@@ -858,7 +868,9 @@ __global__ __launch_bounds__(128 * RW, RW > 2 ? 2 : 1) void wide_kernel(AttnArgs
         }
         if (quad == 0 && row < nrows)
             a.ml[qrow(row) * nsplit + split] = float2{M, f0 * l[r] + f1 * s_l[rw][r][col]};
+        fence();  // LDS serves a wave's accesses in order
         __builtin_amdgcn_wave_barrier();
+        fence();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int x = 2 * i + (lane >> 5), to = (rw * RT + r) * kTileRows + x;
