@@ -126,8 +126,9 @@ __global__ __launch_bounds__(kPostThreads) void post_kernel(PostArgs a) {
 // ranked against all: 41 us instead of 12 for 8 x 16385, 271 instead of 18 for 32 x 131101.) Where few hypotheses lead,
 // or all agree on the tokens, the merge's bound by lists lets through all of their candidates; a second bound, of groups
 // of those, leaves a sort's worth or little more (32 x 131072 logits whose best ones are neighbours: 315 us when found one
-// after the other, 17 so). What finds them one after the other is left for more equal values than LDS takes (32 rows of
-// 131072 equal logits: 415 us).
+// after the other, 17 so). What finds them one after the other is left for more candidates than LDS takes: equal ones (32 rows
+// of 131072 equal logits: 418 us) and, in select, a row's best logits that all lie in few of the 64 groups but in more than
+// one: at 2 to B - 1 residues of the index modulo 64 (8 x 16385: 30 us, 12 for random logits; 32 x 131072: 109, 19).
 // Ordering key of a logit: (sortable(x) << 32) | (0xffffffff - index): a larger key is a larger logit, then a lower index.
 constexpr int kKeep = 32;       // hypotheses at most, so candidates kept per list
 // Logits of a lane: of 8, 10, 12 and 16 the fewest were the fastest (4 x 4096 9.3, 9.4, 9.6, 9.8 us; 32 x 131101 18.3, 18.3,
@@ -135,7 +136,7 @@ constexpr int kKeep = 32;       // hypotheses at most, so candidates kept per li
 constexpr int kPerLane = 8;
 constexpr int kPiece = 64 * kPerLane;  // logits of a wave
 constexpr int kPickWaves = 16;  // waves of a select block at most, a power of two
-constexpr int kGather = 256;    // candidates that are gathered; more (equal ones) take the slow way
+constexpr int kGather = 256;    // candidates that are gathered; more take the slow way
 constexpr int kMergeThreads = 1024;
 constexpr int kMergeWaves = kMergeThreads / 64;
 constexpr int kMergeLists = 1024;  // lists that reach the bound
@@ -509,7 +510,7 @@ __global__ __launch_bounds__(kMergeThreads) void pick_merge_kernel(PickArgs a) {
                     best = sort64(best);
                 }
             }
-        } else {  // many equal ones: the best of all that come after the last one, again and again
+        } else {  // more than that: the best of all that come after the last one, again and again
             Cand last = {~0ull, 0};
             for (int k = 0; k < a.B; ++k) {
                 Cand next = none;

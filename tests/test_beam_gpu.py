@@ -869,6 +869,24 @@ def test_pick_uneven(V, B, dev):
             check_pick(s, want, V)
 
 
+@pytest.mark.parametrize("residues", [2, 3, 16, 31, 32, 63])
+@pytest.mark.parametrize("B,V", [(4, 8192), (32, 8192), (32, 40001)])
+def test_pick_best_tokens_at_few_residues(B, V, residues, dev):
+    """The best tokens, all different, at a few residues of the index modulo 64: more candidates than are gathered."""
+    g = torch.Generator().manual_seed(V + residues)
+    high = torch.zeros(64, dtype=torch.bool)
+    high[torch.randperm(64, generator=g)[:residues]] = True
+    x = torch.stack([torch.randperm(V, generator=g) for _ in range(B)]).float() / V
+    x[:, high[torch.arange(V) % 64]] += 8.0
+    for lead in (0.0, 0.4):
+        st, s = pick_state(dev, B, 16, 9, V + B)
+        st["score"] = (-lead * np.arange(B)[::-1] - 0.37 * (np.arange(B) % 3)).astype(np.float32)
+        s["score"].copy_(torch.tensor(st["score"]))
+        want = OB.pick(x.double().numpy(), *(st[k] for k in ORDER[:6]), V - 1, 0)
+        beam.pick(x.to(dev), *(s[k] for k in ORDER), END_IDX=V - 1)
+        check_pick(s, want, V)
+
+
 @pytest.mark.parametrize("dt", [torch.float32, F16, BF16])
 @pytest.mark.parametrize("B,V,T,step,done", [(1, 1, 1, 0, ()), (1, 700, 4, 3, ()), (4, 4096, 40, 7, (2,)),
                                              (8, 16385, 600, 599, (0, 5)), (32, 5000, 1025, 1000, (1, 2, 30)),
