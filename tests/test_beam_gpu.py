@@ -1136,3 +1136,75 @@ def test_beam_search_of_a_decoder(q8, dev):
         total.append(lp)
     # fp16 activations over two layers in both paths, int8 caches in one of them
     assert np.allclose(search.score.cpu().numpy(), total, atol=0.15 if q8 else 0.05), (search.score, total)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_beam_search_step_by_step(q8, dev):
+    """The same decoder, every captured step against the oracle's selection from the logits that the step itself made and
+    the states before it; with an end token that some hypotheses take on the way."""
+    B, T, V = 5, 9, 300
+    cfg = decode.Config(L=2, H=256, NH=4, NKV=2, inter=512, S=64, n_audio=V, vocab=400)
+    w = decode.random_weights(cfg, 5, dev)
+    prompt = [11, 5, 140]
+    one = decode.DecodeStep(cfg, w, device=dev)
+    first = prefill.Prefill(cfg, w, one.kc, one.vc, one.cos, one.sin, max_T=16).run(prompt)
+    head = (w["head"][0].float() * w["head"][1].float()[:, None]).contiguous()
+    first = (first.float() @ head.t()).expand(B, -1).contiguous()
+    ids = torch.arange(V, device=dev) + 40
+    plen, spos = i64(dev, len(prompt)), i64(dev, 0)
+    kc, vc = one.kc, one.vc
+    cache = lambda: torch.full((cfg.L, B, 2, T, HD), float("nan"), device=dev, dtype=F16)  # noqa: E731
+    layer = lambda c, i: c[i]  # noqa: E731
+    if q8:
+        kc, vc = kv8.empty(*one.kc.shape, device=dev), kv8.empty(*one.kc.shape, device=dev)
+        kv8.quantize(one.kc, one.vc, kc, vc, n=len(prompt))
+        cache = lambda: kv8.empty(cfg.L, B, 2, T, HD, device=dev)  # noqa: E731
+        layer = lambda c, i: (c[0][i], c[1][i])  # noqa: E731
+    ks, vs = cache(), cache()
+    zz = lambda n: torch.zeros(B, n, device=dev, dtype=F16)  # noqa: E731
+    x, h, y, q, o, act, a, d = (zz(n) for n in (256, 256, cfg.n_in, 512, 512, 512, 256, 256))
+    logits = torch.zeros(B, V, device=dev)
+
+    def step(search):
+        prefill.embed_ln_rows(search.tok, w["emb"][0], w["emb"][1], w["ln"][0], x, h, cfg.eps)
+        for i in range(cfg.L):
+            mm_int4.mm_int4(h, *w["w_in"][i], out=y)
+            beam.post(y, spos, plen, one.cos, one.sin, layer(ks, i), layer(vs, i), q, act, NH=4, NKV=2, HD=HD,
+                      ROPE=cfg.sliding[i])
+            beam.attn(q, layer(kc, i), layer(vc, i), plen, layer(ks, i), layer(vs, i), spos, o, HD ** -0.5,
+                      src=search.src)
+            mm_int4.mm_int4(o, *w["w_o"][i], out=a)
+            mm_int4.mm_int4(act, *w["w_down"][i], out=d)
+            prefill.add_ln_rows(x, a, d, w["norm"] if i == cfg.L - 1 else w["ln"][i + 1], h, B, cfg.eps)
+        torch.matmul(h.float(), head.t(), out=logits)
+        search(logits)
+        fused.pos_advance(spos)
+
+    # a first search tells which token some hypothesis takes as its fourth one: in the second it is the end
+    end = 40
+    for captured in (False, True):
+        search = beam.BeamSearch(B, T, ids, end_id=end, min_new=2)
+        if captured:
+            search(first)
+            step(search)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                step(search)
+            search.reset()
+        spos.zero_()
+        for t in range(T):
+            before = [getattr(search, k).cpu().numpy().copy() for k in ORDER[:6]]
+            before[3] = int(before[3][0])
+            if t == 0:
+                search(first)
+            elif captured:
+                graph.replay()
+            else:
+                step(search)
+            torch.cuda.synchronize()
+            want = OB.pick((logits if t else first).double().cpu().numpy(), *before, end - 40, 2, ids=ids.cpu().numpy())
+            check_pick({k: getattr(search, k) for k in ORDER}, want, V)
+        if captured:
+            assert search.done.any() and search.lens.min() < T
+        end = int(search.hist[0, 3])
