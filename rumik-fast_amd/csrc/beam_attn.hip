@@ -501,12 +501,19 @@ RK_DEV Slots suffix_slots(const AttnArgs& a, int b, int g) {
 
 // Small caches, in one launch and without a workspace: a block takes all slots of one hypothesis and KV head, its eight
 // waves shared out between prefix and suffix by their lengths, and writes the result. A step costs a wave about 2 us of
-// memory latency, and a CU holds one such block. So it pays for one step per wave and two blocks per CU; with about as
-// many blocks as CUs, where part_kernel has few blocks to a hypothesis, for three. In a graph, part_kernel and join_kernel
-// / this: 4 hypotheses and 4 KV heads x (34 + 9) slots 6.7 / 5.6 us, x (300 + 70) 7.6 / 9.0; with 8 KV heads 16 x (300 +
-// 70) 8.9 / 8.8, x (500 + 260) 11.8 / 12.3; 32 x (100 + 20) 11.3 / 6.2, x (500 + 260) 17.6 / 12.8, x (1024 + 100) 16.2 /
-// 17.0; 64 x (190 + 60) 17.1 / 12.8, x (700 + 50) 21.3 / 22.1; 128 x (190 + 60) 20.3 / 25.1. An eager call saves a launch
-// besides.
+// memory latency, and a CU holds one such block. So it pays for one step per wave and two blocks per CU; for half as many to
+// as many blocks as CUs, where part_kernel has few blocks to a hypothesis, for three, at 128 of them about even. In a graph,
+// part_kernel and join_kernel / this, 4 query heads per KV head, plain, then both caches int8:
+//   one step   4 hypotheses and 4 KV heads x (34 + 9) slots 7.3 / 5.7 us, 8.3 / 6.9; with 8 KV heads 32 x (100 + 20) 11.0 /
+//              6.2, 11.8 / 7.2; 64 x (190 + 60) 16.7 / 12.6, 17.4 / 13.6; but 68 x (34 + 9) 15.2 / 13.4, 16.9 / 17.6, and
+//              128 x (190 + 60) of one head 16.2 / 24.3, 18.1 / 27.7
+//   three      with 8 KV heads 16 x (200 + 80) 8.9 / 7.9, 9.2 / 9.1, x (500 + 260) 11.9 / 12.1, 11.2 / 12.8, x (700 + 68)
+//              11.5 / 12.5, 11.0 / 12.8, x (100 + 660) 15.4 / 12.2, 15.9 / 12.8; 18 x (500 + 260) 14.6 / 12.2, 14.7 / 12.8,
+//              x (700 + 68) 12.6 / 12.5, 11.8 / 12.7, x (100 + 660) 13.3 / 12.3, 14.2 / 12.8; 32 x (500 + 260) 17.5 / 12.6,
+//              17.5 / 13.3, x (100 + 660) 19.7 / 12.7, 20.2 / 13.4; 34 x (500 + 260) 20.5 / 22.9, 20.4 / 23.7. It loses where
+//              part_kernel takes a long prefix in full groups of 16 rows: 32 x (700 + 68) of one head per KV head 10.2 / 13.7,
+//              10.3 / 14.8
+// An eager call saves a launch besides.
 constexpr int kDirectWaves = 8;
 constexpr int kDirectSlots = kDirectWaves * kStep;
 RK_DEV int direct_waves(int n1, int n2) {  // the prefix's: its share of the steps n1 + n2, but one at least for either

@@ -301,6 +301,19 @@ def test_attn_around_one_launch(dt, p8, s8, dev):
         run_and_check(attn_case(dev, dt, 2, 1, 2, 0, n, None, [n - 1], False, s8, seed=n), dt)
 
 
+@pytest.mark.parametrize("dt,p8,s8", [(F16, False, False), (BF16, True, True)])
+@pytest.mark.parametrize("B,nkv", [(127, 1), (64, 2), (128, 2), (257, 1)])
+def test_attn_around_one_launch_of_three_steps(dt, p8, s8, B, nkv, dev):
+    """127, 128, 256 and 257 pairs of hypothesis and KV head: one launch for up to 768 slots from 128 pairs to 256."""
+    for S, T in ((300, 468), (300, 469)):
+        c = attn_case(dev, dt, B, nkv, 1, S, T, S - 1, [T - 1 - b % 7 for b in range(B)], p8, s8, seed=S + T)
+        c["run"]()
+        rows = [0, 1, B // 2, B - 1]
+        kv = c["kv"]
+        check_attn(c["o"][rows], c["q"][rows], lambda b, h: kv(rows[b], h), dt, c["scale"], c["unit"])
+        assert bool(torch.isfinite(c["o"]).all())
+
+
 @pytest.mark.parametrize("dt,p8,s8", KINDS)
 @pytest.mark.parametrize("B,rows,T,seed", [(4, 4, 40, 0), (6, 9, 131, 1), (8, 3, 17, 2)])
 def test_attn_table(dt, p8, s8, B, rows, T, seed, dev):
