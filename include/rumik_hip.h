@@ -526,8 +526,8 @@ int rk_beam_post(const void* y, int ldy, const int64_t* spos, int nspos, const i
  * suffix slot. Suffix slot t of hypothesis b is slot t of row src[b * src_ld + t] (src NULL: row b); an entry outside
  * [0, rows) is no slot. A hypothesis without any slot, or whose scores are all -inf, gets zeros. What lies in other slots
  * does not matter, NaN included. fp32 scores, softmax and sums; weights are rounded to dt before they meet V (fp16: 2^-11
- * relative, or 2^-32 of the largest weight where that is more; bf16: 2^-8), in an int8 part to fp16 with V's scale in them
- * (2^-11 relative, or 2^-31 of the part's largest |V| where that is more).
+ * relative, or 2^-32 of the largest weight where that is more; bf16: 2^-8), in an int8 part with V's scale in them, to
+ * 2^-21 where dt is fp16, 2^-11 where it is bf16 (or to 2^-31 of the part's largest |V| where that is more).
  * kc NULL: no prefix; ks NULL: no suffix (one of them is needed). With kc_scale / vc_scale [NKV, S], ks_scale /
  * vs_scale [rows, NKV, T] that part is int8. ws: rk_beam_attn_ws_bytes(B, NH, NKV, S, T) bytes (S or T 0 for a part
  * that is absent), contents irrelevant; calls that may overlap need workspaces of their own. HD = 128, NH / NKV in

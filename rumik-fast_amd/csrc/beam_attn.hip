@@ -6,9 +6,16 @@
 // consecutive slots per lane, which is how the next product, O^T = V^T P^T, wants P if its k index runs over the slots in
 // the order 4 quad + (0..3), 16 + 4 quad + (0..3): the weights stay in their lanes. The softmax is in log2 units with a
 // running maximum that moves only when a score exceeds it by more than 2^kSlack, so the exchange between the quads and
-// the rescaling of O run in few steps. Scores, statistics and sums are fp32. P is rounded to the operands' type (fp16:
-// 2^-11 relative, or 2^-32 of the largest weight where that is more, bf16: 2^-8 relative; as much again as the output's own
-// rounding). int8 caches run on fp16 operands, in which the codes are exact; K's scale goes to the scores, V's scale to P.
+// the rescaling of O run in few steps. Scores, statistics and sums are fp32. int8 caches run on fp16 operands, in which the
+// codes are exact; K's scale goes to the scores, V's scale to P.
+//
+// P's rounding. Plain caches: to their type, fp16 2^-11 relative, or 2^-32 of the largest weight where that is more, bf16 2^-8;
+// the sum is of the rounded weights, so what they have in common cancels, and the result is 1.0 to 1.3 times as far off as by
+// its own rounding to the type. In two 16-bit parts, with a product of V for each, it would be 1.0 times, for 82 us instead
+// of 73 (32 hypotheses x 65536 slots, 8 KV heads): not taken. int8: the scales are in P, nothing cancels, and a result in fp16
+// was up to 1.6 times as far off. There P has two parts of fp16, 22 bits: 1.0 times, for 97.8 us instead of 86.5 (128 rows x
+// 65536 slots and 8 heads), 74.5 instead of 67.0 (64 rows), 19.4 instead of 19.1 (5 hypotheses x 30001). With bf16
+// activations one part of fp16 does: 1.0 times.
 //
 // Launches: direct_kernel alone for small caches; else part_kernel for the suffixes and short prefixes, wide_kernel for
 // long prefixes of many query rows and join_kernel, which adds the splits up. All read the lengths on the device; a
@@ -93,6 +100,17 @@ RK_DEV uint32_t codes2_to_h2(uint32_t w) {
 RK_DEV u2_t codes4_to_h4(uint32_t w) {
     return u2_t{codes2_to_h2(perm(0u, w, 0x0c010c00u)), codes2_to_h2(perm(0u, w, 0x0c030c02u))};
 }
+
+// The weights of 8 slots as they meet V; TWO (int8 with fp16 activations): hi + lo. (An infinite V, which codes do not have,
+// would meet a lo of 0.)
+template <bool TWO>
+struct Weights {
+    u4_t hi;
+};
+template <>
+struct Weights<true> {
+    u4_t hi, lo;
+};
 
 // A wave's state for RT tiles of 16 query rows; lane (col, quad) = (lane & 15, lane >> 4): query row col of each tile.
 template <int RT>
@@ -193,8 +211,8 @@ RK_DEV void scale_weights(float (&vw)[8], State<RT>& s) {
 // maximum (32 at 2^29), and no longer 0. ok: bit i set where slot i is one. The sum is of the rounded weights, those
 // that meet V, by one more product with ones (the VALU is the busier unit); int8's weights meet V with its scales in them,
 // there it is of the fp32 ones.
-template <bool BF16, bool Q8, bool MASK, int RT>
-RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)[8], uint32_t ok, State<RT>& s, int r) {
+template <bool BF16, bool Q8, bool TWO, bool MASK, int RT>
+RK_DEV Weights<TWO> weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)[8], uint32_t ok, State<RT>& s, int r) {
 #pragma clang fp contract(off)
     float t[8];
     float top = kLowest;  // as it is, no product of it: a lane without a slot is below any score
@@ -216,21 +234,29 @@ RK_DEV u4_t weights(const f4_t (&sc)[2], const float (&ks)[8], const float (&vw)
 #pragma unroll
         for (int d = 0; d < 8; ++d) s.acc[r][d] *= f;
     }
+    // (without it the tiles' work is interleaved, and blocks of 128 rows spill 120 bytes: 101 us instead of 98)
+    if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(t[i] - s.m[r]);
-    u4_t w;
+    Weights<TWO> w;
     if constexpr (Q8) {
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += t[i];
         s.l[r][0] += sum;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2<false>(t[2 * i] * vw[2 * i], t[2 * i + 1] * vw[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            const float x = t[2 * i] * vw[2 * i], y = t[2 * i + 1] * vw[2 * i + 1];
+            w.hi[i] = pack2<false>(x, y);
+            if constexpr (TWO)
+                w.lo[i] = pack2<false>(__builtin_fmaf((float)as_h2(w.hi[i]).x, -1.0f, x),
+                                       __builtin_fmaf((float)as_h2(w.hi[i]).y, -1.0f, y));
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2<BF16>(t[2 * i], t[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) w.hi[i] = pack2<BF16>(t[2 * i], t[2 * i + 1]);
         const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
-        s.l[r] = mfma<BF16>(u4_t{one, one, one, one}, w, s.l[r]);
+        s.l[r] = mfma<BF16>(u4_t{one, one, one, one}, w.hi, s.l[r]);
     }
     return w;
 }
@@ -359,8 +385,8 @@ RK_DEV void products(const Step<Q8>& st, const State<RT>& s, f4_t (&sc)[RT][2]) 
 }
 
 // Their softmax: the weights w of each tile.
-template <bool BF16, bool Q8, bool MASK, class Loaded, int RT>
-RK_DEV void softmax(const Loaded& st, const f4_t (&sc)[RT][2], State<RT>& s, u4_t (&w)[RT]) {
+template <bool BF16, bool Q8, bool MASK, class Loaded, bool TWO, int RT>
+RK_DEV void softmax(const Loaded& st, const f4_t (&sc)[RT][2], State<RT>& s, Weights<TWO> (&w)[RT]) {
     float vw[8];
     if constexpr (Q8) {
 #pragma unroll
@@ -368,13 +394,13 @@ RK_DEV void softmax(const Loaded& st, const f4_t (&sc)[RT][2], State<RT>& s, u4_
         scale_weights(vw, s);
     }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) w[r] = weights<BF16 && !Q8, Q8, MASK>(sc[r], st.ks, vw, st.ok, s, r);
+    for (int r = 0; r < RT; ++r) w[r] = weights<BF16 && !Q8, Q8, TWO, MASK>(sc[r], st.ks, vw, st.ok, s, r);
 }
 
 // The weights' products with the step's V, transposed to the A operand (row = dim, k = slot): dim 8 col + d of the
 // eight slots at a time.
-template <bool BF16, bool Q8, bool MASK, int RT>
-RK_DEV void add_values(const Step<Q8>& st, const u4_t (&w)[RT], State<RT>& s) {
+template <bool BF16, bool Q8, bool MASK, bool TWO, int RT>
+RK_DEV void add_values(const Step<Q8>& st, const Weights<TWO> (&w)[RT], State<RT>& s) {
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
         u4_t vt;
@@ -394,14 +420,17 @@ RK_DEV void add_values(const Step<Q8>& st, const u4_t (&w)[RT], State<RT>& s) {
             }
         }
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s.acc[r][d] = mfma<BF16 && !Q8>(vt, w[r], s.acc[r][d]);
+        for (int r = 0; r < RT; ++r) {
+            if constexpr (TWO) s.acc[r][d] = mfma<BF16 && !Q8>(vt, w[r].lo, s.acc[r][d]);
+            s.acc[r][d] = mfma<BF16 && !Q8>(vt, w[r].hi, s.acc[r][d]);
+        }
     }
 }
 
 template <bool BF16, bool Q8, bool MASK>
 RK_DEV void take(const Step<Q8>& st, State<1>& s) {
     f4_t sc[1][2];
-    u4_t w[1];
+    Weights<!BF16 && Q8> w[1];
     products<BF16>(st, s, sc);
     softmax<BF16, Q8, MASK>(st, sc, s, w);
     add_values<BF16, Q8, MASK>(st, w, s);
@@ -747,7 +776,7 @@ __global__ __launch_bounds__(128 * RW, RW > 2 ? 2 : 1) void wide_kernel(AttnArgs
     // earlier, in front of phase 2 i that of tile i + 1.
     constexpr bool kB = BF16 && !Q8;  // int8 runs on fp16 operands
     f4_t sc[RT][2];
-    u4_t w[RT];
+    Weights<!BF16 && Q8> w[RT];
     auto refill = [&](int i) {  // in phase 2 i + 1
         if (i > 0) issue(begin + (i - 1 + TL::kCount) * stride, (uint32_t)(i - 1) % TL::kCount);
     };

@@ -689,6 +689,53 @@ def test_attn_many_low_weights(dt, p8, s8, B, nkv, rep, S, T, depth, dev):
     assert bool((off <= tol).all()), (float((off / tol).max()), float((off / mag).max()))
 
 
+@pytest.mark.parametrize("B,nkv,rep,S,T", PATHS)
+def test_attn_int8_weights_of_fp16(B, nkv, rep, S, T, dev):
+    """Slots in pairs of nearly the same score and opposite V: a result far below its terms, which shows the weights' own
+    roundings; with int8 caches and fp16 activations 2^-21 relative at most, and within 2^-32 of twice the largest V scale for
+    codes to 127. The scores have one product: off by |s| 2^-22 (three roundings; a tenth of the weights at most has |s| > 9,
+    and next to no weight), exp by 2^-21."""
+    plen, slen = S - 2, T - 2
+    c = attn_case(dev, F16, B, nkv, rep, S, T, plen, [slen - 1], True, True, seed=S, junk=0.0)
+    g = torch.Generator(device=dev).manual_seed(S + 1)
+    c["q"].zero_()
+    c["q"].view(B, -1, HD)[..., 0] = 1.0
+    for key, value, n in (("kc", "vc", S // 2), ("ks", "vs", T // 2)):
+        lead = c[key][0].shape[:-2]
+        score = -(8 if n < 2000 else 100) * torch.rand(*lead, n, device=dev, generator=g) - 0.5
+        score = torch.stack((score, score * (1 - 2.0 ** -7 * torch.rand(*lead, n, device=dev, generator=g))), -1).flatten(-2)
+        k = torch.zeros(*lead, 2 * n, HD, dtype=torch.int8, device=dev)
+        k[..., 0] = -64
+        v = torch.randn(*lead, n, HD, device=dev, generator=g).to(F16)
+        c[key] = (k, (score / -64).contiguous())
+        c[value] = as_cache(torch.stack((v, -v), -2).flatten(-3, -2).contiguous(), True)[0]
+    beam.attn(c["q"], c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], 1.0)
+    want, mag = attend64(c["q"], [dense(c[k])[:, :plen] for k in ("kc", "vc")],
+                         [dense(c[k])[:, :, :slen] for k in ("ks", "vs")], 1.0)
+    n, most = plen + slen, max(x[1].max().item() for x in (c["vc"], c["vs"]))
+    tol = (2 * (2.0 ** -21 + 2.0 ** -21 + 9.1 * 2.0 ** -22) + (n / 32 + 64) * U[torch.float32]) * mag + \
+        n * 2.0 ** -32 * 2 * most * 127 + U[F16] * want.abs() + 2.0 ** -25
+    off = (c["o"].double().view_as(want) - want).abs()
+    assert bool((off <= tol).all()), (float((off / tol).max()), float((off / mag).max()))
+
+
+@pytest.mark.parametrize("B,nkv,rep,S,T", PATHS)
+def test_attn_int8_one_slot_that_counts(B, nkv, rep, S, T, dev):
+    """One slot outweighs all others by e^60: with fp16 activations the result is its V row, rounded once."""
+    c = attn_case(dev, F16, B, nkv, rep, S, T, S, [T - 1], True, True, seed=S, junk=0.0)
+    c["q"].zero_()
+    c["q"].view(B, -1, HD)[..., 0] = 1.0
+    for k in (c["kc"], c["ks"]):
+        k[0].zero_()
+    at = S * 2 // 3
+    c["kc"][0][:, at, 0] = 60
+    c["kc"][1][:, at] = 1.0
+    beam.attn(c["q"], c["kc"], c["vc"], c["plen"], c["ks"], c["vs"], c["spos"], c["o"], 1.0)
+    want = dense(c["vc"])[:, at].repeat_interleave(rep, 0).expand(B, -1, -1).reshape(B, -1)
+    off = (c["o"].double() - want).abs()
+    assert bool((off <= (U[F16] + 2.0 ** -20) * want.abs() + 2.0 ** -25).all()), float((off / want.abs()).max())
+
+
 @pytest.mark.parametrize("p8", [False, True])
 def test_attn_matches_the_one_row_attention(p8, dev):
     """A hypothesis by itself is fused.attn over one cache holding its prefix and suffix."""
