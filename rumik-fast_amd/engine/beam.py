@@ -1,4 +1,4 @@
-"""Several hypotheses of one prompt (beam search, best of n) decoded side by side on MI355X: what stands between the
+"""Several hypotheses of one prompt decoded side by side on MI355X, as a beam search does: what stands between the
 projections of such a step. The reference decodes one sequence (engine/rumik_fused.py:97-121); there post, the decode
 attention and the sampler take one row, here B.
 
@@ -11,7 +11,8 @@ activations' type or an int8 pair (codes, scales) as in kv8. A step of B hypothe
     beam.attn(q, kc, vc, plen, ks, vs, spos, o, scale, src=search.src)
     ... mm_int4(o, *w_o), mm_int4(act, *w_down), add_ln over the rows
 
-then the head, `search(logits)` and `fused.pos_advance(spos)`. `plen` (the prompt's length) and `spos` (the newest
+then the head, `search(logits)` and `fused.pos_advance(spos)`. (The head's product for B rows and, for best of n instead of
+a search, the sampling are the caller's.) `plen` (the prompt's length) and `spos` (the newest
 token's suffix slot, one for all or one each) are int64 on the device, so that one captured graph serves every step.
 Reordering hypotheses moves no cache: pick permutes the table src, through which attn finds a hypothesis's slots in
 the rows that wrote them.
@@ -218,9 +219,9 @@ def pick(logits, score, done, lens, step, hist, src, tok, parent, END_IDX, MIN_N
 
 class BeamSearch:
     """A search's states on the device (score, done, lens, step, hist, src, tok, parent) and its workspace; `__call__`
-    picks from logits [B, len(audio_ids)] in place, as sample.FusedSampler does for one sequence. tok is the next step's
-    input, hist[:, :step] the hypotheses' tokens, src what beam.attn takes. hist and src have T columns, as the suffix
-    caches have slots."""
+    picks from logits [B, len(audio_ids)] in place, as sample.FusedSampler samples for one sequence (but without its stop
+    predictor: end_id alone ends a hypothesis). tok is the next step's input, hist[:, :step] the hypotheses' tokens, src
+    what beam.attn takes, score the sum of log probabilities. hist and src have T columns, as the suffix caches have slots."""
 
     def __init__(self, B, T, audio_ids, end_id, min_new=0, device=None):
         dev = audio_ids.device if device is None else torch.device(device)
