@@ -612,7 +612,8 @@ __global__ __launch_bounds__(kThreads, 2) void part_kernel(AttnArgs a) {
 // the block's rows. 16-byte chunk c of a row of 256 bytes is stored at chunk c ^ (row & 15), so that the K operands (16
 // rows, one chunk) touch every bank equally often. An int8 tile is stored as it comes and converted once for all the
 // block's waves, by one half of them K, by the other V, into two pairs of tiles of fp16 that are laid out like plain ones
-// (8 heads x 65536 slots, 128 rows: 85 us, 91 with each wave converting what it reads; 64 rows 68 and 71).
+// (8 heads x 65536 slots, one product with V per weight, 128 rows: 85 us, 91 with each wave converting what it reads; 64
+// rows 68 and 71).
 constexpr int kRing = 4, kRing8 = 5;
 
 template <bool Q8>
@@ -977,10 +978,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
 
 // A long prefix goes to the wide kernel, which reads it once, from so much work on (slots x KV heads x groups of 16 rows)
 // that reading it once per group from L2 takes longer than the wide kernel's extra launch and its larger start. In a
-// graph, part_kernel against wide_kernel, 8 KV heads, plain: 20 rows x 10000 slots 19.4 / 19.9 us, x 30000 41 / 31; 64 x
-// 4096 18.4 / 20.1, x 10000 31 / 22.6; 128 x 2500 21.9 / 21.0, x 30000 138 / 44. int8 (half the bytes, but codes
-// to convert and scales to apply): 32 x 30000 28.5 / 33, 48 x 65536 67 / 70; 80 x 30000 55 / 55; 128 x 10000
-// 34 / 36, x 20000 57 / 47.
+// graph, part_kernel against wide_kernel, 8 KV heads, plain: 20 rows x 10000 slots 19.7 / 19.5 us, x 30000 41 / 31; 64 x
+// 4096 18.2 / 19.9, x 10000 31 / 22.0; 128 x 2500 22.0 / 22.4, x 30000 138 / 45. int8 (half the bytes, but codes
+// to convert and scales to apply), bf16 and fp16 activations: 32 x 30000 27 / 40, 28 / 42; 48 x 65536 66 / 68, 66 / 73; 64 x
+// 30000 44 / 43, 44 / 45, x 65536 83 / 69, 84 / 75; 80 x 30000 53 / 50, 53 / 56; 128 x 10000 34 / 35, 35 / 37, x 20000
+// 56 / 47, 56 / 51.
 constexpr long long kWideWork = 3 << 16, kWideWork8 = 1 << 20;
 constexpr long long kWideMin = 1024;  // and none shorter, whatever the number of heads
 constexpr int kWideRows = kTileRows, kWideRows8 = 3 * kTileRows;  // for more rows than these
