@@ -566,6 +566,9 @@ int rk_beam_attn_params_size(void);
  *   lens = parent's, + 1 unless the parent had ended; hist and src [B, T]: columns t < step of row k become those of
  *   row parent[k], column step becomes tok[k] (hist) and k (src: the row that slot `step` is about to be written to, as
  *   rk_beam_post does), later columns are left as they were; step + 1.
+ * Values are formed in 64 bits from an fp32 sum of exponentials: candidates of two hypotheses within 2^-18 of each other may
+ * come in either order, and of a hypothesis with a score below -2^50 (as the type's lowest value for a mask leaves it), whose
+ * tokens 64 bits no longer tell apart, any may be taken.
  * With fewer than B candidates above -inf the others end: parent = k, tok of end_idx, score -inf, done.
  * step outside [0, T): nothing is written. The *_out tensors may be the inputs themselves (in place) or others, but must
  * not overlap them otherwise. Start: score = 0 for one hypothesis and -inf for the others, done = 0, lens = 0, step = 0.
