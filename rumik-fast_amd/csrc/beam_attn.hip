@@ -234,7 +234,8 @@ RK_DEV Weights<TWO> weights(const f4_t (&sc)[2], const float (&ks)[8], const flo
 #pragma unroll
         for (int d = 0; d < 8; ++d) s.acc[r][d] *= f;
     }
-    // (without it the tiles' work is interleaved, and blocks of 128 rows spill 120 bytes: 101 us instead of 98)
+    // A bound for the compiler: without it the work of several tiles is interleaved, and blocks of 128 rows spill 120 bytes (128
+    // fp16 rows x 65536 slots, 8 heads: 101 us instead of 98).
     if constexpr (Q8) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(t[i] - s.m[r]);
